@@ -281,7 +281,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows16_kernel(AttnArgs a) {
   float m = -INFINITY, l = 0.f;
 
   // `all`: every row sees all of these keys
-  auto compute = [&](int pos, const T& x, uint32_t there, auto all) {
+  auto compute = [&](int pos, T& x, uint32_t there, auto all) {
     constexpr bool kAll = decltype(all)::value;
     f32x4 s[2];
 #pragma unroll
@@ -333,8 +333,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows16_kernel(AttnArgs a) {
       p[2 * u + 1] = pack2<TYPE>(s[u][2], s[u][3]);
     }
 
-    // scales of this lane's keys: zeros behind the end, and finite stand-ins for NaN blocks (byte 255: the byte of
-    // ~vs is 0)
+    // scales of this lane's keys: zeros behind the end, and zeros of a finite scale for NaN blocks (byte 255: the byte of
+    // ~vs is 0; in mxfp8 their codes may be NaN under every scale)
     uint32_t vs[2] = {x.vs[0], x.vs[1]};
     if constexpr (!kAll) {
 #pragma unroll
@@ -353,6 +353,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows16_kernel(AttnArgs a) {
         if ((vs[e >> 2] & at) == at) {
           nan |= 1u << e;
           vs[e >> 2] &= ~at;
+          if constexpr (FMT == kMxFp8)
+#pragma unroll
+            for (int i = 0; i < T::kVWords; ++i) x.v[e >> 2][e & 3][i] = 0u;
         }
       }
       float poison = 0.f;
@@ -603,9 +606,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(AttnArgs a) {
         byte = 0u;
         w[e] = u32x2{0u, 0u};
       }
-      if (byte == 255u) {
+      if (byte == 255u) {  // in mxfp8 the codes may be NaN under every scale
         nan |= 1u << e;
         byte = 0u;
+        if constexpr (FMT == kMxFp8) w[e] = u32x2{0u, 0u};
       }
       vscale[e] = mx_scale(byte);
     }

@@ -347,3 +347,60 @@ def test_refusals(gpu):
         c.attend(q, table.long(), *good[1:])
     c.write(k[:0], k[:0], slots[:0])
     assert c.attend(q[:0], table[:0], i32([]), i32([0]), 0).shape == (0, 4, 64)
+
+
+def _poisoned_and_clean(b, clean, spots, new, group):
+    """Outputs over a cache with NaN blocks and over the same one without, and where the first must be NaN.  ``spots``:
+    (sequence, position, block of the head or None for the key)."""
+    heads, dim = b.cache.heads, b.cache.head_dim
+    q, _, o = b.attend(new, group)
+    _, _, c = clean.attend(new, group, q=q)
+    want = torch.zeros(sum(new), heads, group, dim, dtype=torch.bool)
+    for i, pos, head, block in spots:
+        a = sum(new[:i])
+        sees = a + torch.nonzero(b.lens[i] - new[i] + torch.arange(new[i]) >= pos).flatten()
+        if block is None:
+            want[sees, head] = True
+        else:
+            want[sees, head, :, 32 * block: 32 * block + 32] = True
+    return o.cpu(), c.cpu(), want.flatten(1, 2)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 30, 40, 200])
+def test_attend_nan_blocks_in_each_format(gpu, bad, fmt, dtype, dim, new):
+    """16-row tiles (1 and 30 new tokens) and 128-row ones: NaN exactly where a row sees the key or the value block; all
+    else is bit for bit what it is without them, in the tile that holds them too."""
+    n = 260
+    p_k, p_v = n - 3, n - 20
+    b, clean = (_Batch(gpu, [n], 2, dim, 16, fmt, dtype) for _ in range(2))
+    b.k[p_k, 0, 3], b.v[p_v, 1, 40], b.v[p_v + 9, 1, 7] = bad, bad, bad
+    o, c, want = _poisoned_and_clean(b.fill(), clean.fill(), [(0, p_k, 0, None), (0, p_v, 1, 1), (0, p_v + 9, 1, 0)],
+                                     [new], 2)
+    assert torch.equal(o.isnan(), want) and torch.equal(o[~want], c[~want])
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+def test_attend_nan_blocks_in_the_largest_tiles(gpu, fmt):
+    """256 rows a work-group, as above."""
+    lens, new = [300] * 16, [70] * 16
+    b, clean = (_Batch(gpu, lens, 8, 128, 32, fmt, torch.bfloat16) for _ in range(2))
+    b.v[5 * 300 + 270, 3, 100], b.k[7 * 300 + 290, 6, 1] = math.nan, math.inf
+    o, c, want = _poisoned_and_clean(b.fill(), clean.fill(), [(5, 270, 3, 3), (7, 290, 6, None)], new, 4)
+    assert torch.equal(o.isnan(), want) and torch.equal(o[~want], c[~want])
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_read_nan_blocks(gpu, fmt, dtype):
+    """A block with a NaN or an infinity reads back as NaN in 16 bits, the other blocks as they are."""
+    b = _Batch(gpu, [40], 2, 64, 16, fmt, dtype)
+    b.k[3, 1, 40], b.k[9, 0, 0], b.v[5, 0, 2], b.v[6, 1, 63] = math.nan, math.inf, -math.inf, math.nan
+    b.fill()
+    for got, x in zip(b.read(), (b.k, b.v)):
+        got, want = got.cpu(), om.values(x, fmt).to(dtype)
+        assert int(want.isnan().sum()) == 64 and torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(), want.nan_to_num())
