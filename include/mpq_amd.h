@@ -728,7 +728,9 @@ int mpq_mx_linear(const void* x, int dtype, int64_t ldx, const uint8_t* x_codes,
  *   k_codes  (pages, heads, page, bytes of dim codes)        k_scales (pages, heads, page, dim / 32)
  *   v_codes  (pages, heads, page / 4, dim / 8, 4, bytes of 8 codes)
  *   v_scales (pages, heads, page / 4, dim / 32, 4)
- * The fourth index of the values is the token within its group of four.
+ * The fourth index of the values is the token within its group of four.  NaN is scale byte 255: the E4M3 codes 0x7f
+ * and 0xff under another scale byte, which mpq_kv_write never stores, are not supported (mpq_kv_attend may let such a
+ * value reach rows that do not see it).
  *
  * mpq_kv_write: tokens x heads x dim keys and values (MPQ_BF16 or MPQ_F16, strides in elements, dim contiguous)
  * into their slots (page * page size + place in the page); a slot outside the pool is skipped, and of two tokens

@@ -13,7 +13,9 @@
 //
 // Positions that a row does not see get -inf; a row that sees nothing is 0 (lse -inf).  Memory behind a sequence's
 // end may hold anything: its scores are replaced and its values read as zeros.  A value block that stands for NaN
-// poisons exactly the rows that see it.
+// (scale byte 255) poisons exactly the rows that see it.  NaN codes of mxfp8 under another scale byte, which the write
+// kernel never stores, would reach every row of their tile; a search for them in each tile took 1 % of chunks over a long
+// context and 12 % of whole prompts (8 of 2048: 465 -> 521 us), so caches must not hold any.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

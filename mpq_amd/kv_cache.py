@@ -51,7 +51,9 @@ class QuantizedKVCache:
     def from_tensors(cls, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
                      v_scales: torch.Tensor, *, fmt: str = "mxfp8",
                      dtype: torch.dtype = torch.bfloat16) -> "QuantizedKVCache":
-        """A cache over tensors that the caller allocated (used in place)."""
+        """A cache over tensors that the caller allocated (used in place).  Where others filled them, NaN is a block's scale
+        byte 255: codes 0x7f and 0xff of ``mxfp8`` under another scale byte are not supported (:meth:`attend` may let
+        them reach rows that do not see them)."""
         self = cls.__new__(cls)
         self._set(k_codes, k_scales, v_codes, v_scales, fmt, dtype)
         return self
