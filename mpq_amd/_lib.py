@@ -299,7 +299,7 @@ def ptr(t) -> Optional[int]:
 def stream_handle(device=None) -> int:
     import torch
 
-    index = getattr(device, "index", None)
-    if index is not None:  # the handle itself, without the stream object around it (2 us of a small call)
-        return torch._C._cuda_getCurrentRawStream(index)
+    # a device of known number: the handle itself, without the stream object around it (2 us of a small call)
+    if isinstance(device, torch.device) and device.type == "cuda" and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
     return int(torch.cuda.current_stream(device).cuda_stream)

@@ -65,3 +65,17 @@ def test_pointer_arguments_stay_alive_until_the_call_returns():
     _lib.call("mpq_last_error_code")
     gc.collect()
     assert ref() is None
+
+
+def test_stream_handle_takes_what_torch_takes(monkeypatch):
+    """Devices as text, numbers, without a number and of another type go to torch; only a numbered ROCm device has the
+    direct way."""
+    import types
+
+    torch = pytest.importorskip("torch")
+    asked = []
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: asked.append(d) or types.SimpleNamespace(cuda_stream=7))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    others = (None, "cuda:0", "cuda", 1, torch.device("cuda"), torch.device("cpu:0"))
+    assert [_lib.stream_handle(d) for d in others] == [7] * len(others) and asked == list(others)
+    assert _lib.stream_handle(torch.device("cuda:1")) == 101 and len(asked) == len(others)
