@@ -752,6 +752,7 @@ int mpq_kv_read(const int32_t* block_table, int64_t batch, int64_t table_width, 
  * Attention of new tokens over the cache that already holds them: q (total_q x q_heads x dim, strides in elements,
  * dim contiguous), sequence i the tokens q_starts[i] to q_starts[i + 1] (at most max_q of them), its keys the
  * positions 0 to kv_lens[i] of its row of block_table.  q_heads / heads query heads share a key/value head.
+ * Tokens before q_starts[0], behind q_starts[batch], or behind max_q of their sequence see nothing; q_starts rises.
  * causal: new token t of n sees the positions up to kv_len - n + t, else all.  out (total_q x q_heads x dim, the
  * type of q), lse (total_q x q_heads fp32, natural logarithm, or NULL).  A row that sees nothing is 0 with lse
  * -inf; positions whose page the table does not name are not seen.  max_kv: an estimate of the longest kv_len

@@ -29,7 +29,7 @@ struct AttnArgs {
   const char* q;
   int64_t q_ts, q_hs;
   int64_t total_q;
-  int q_heads, group;
+  int q_heads, group, batch, max_q;
   const int32_t* table;
   int64_t width;
   const int32_t *kv_lens, *q_starts;
@@ -77,6 +77,8 @@ __device__ __forceinline__ float group_sum(float v) {
 // A sequence as a work-group sees it; lengths from device memory are brought into range first.
 struct Seq {
   int q0, q_len, kv_len;
+  // (new token, query head) pairs of a key/value head
+  __device__ int rows(const AttnArgs& a) const { return min(q_len, a.max_q) * a.group; }
   __device__ Seq(const AttnArgs& a, int b) {
     const int64_t s = min((int64_t)max(a.q_starts[b], 0), a.total_q);
     q0 = (int)s;
@@ -85,6 +87,29 @@ struct Seq {
   }
   __device__ int last_seen(const AttnArgs& a, int t) const { return a.causal ? kv_len - q_len + t : kv_len - 1; }
 };
+
+// Rows of this key/value head that no tile holds see nothing: tokens before the first sequence or behind the last one (a
+// batch padded to a captured size has such) and those of a sequence behind max_q.  By one work-group of each
+// sequence and head (`mine`).
+template <int D>
+__device__ __forceinline__ void clear_unheld(const AttnArgs& a, const Seq& seq, int head, int b, bool mine) {
+  const auto clear = [&](int from, int to) {
+    const int pieces = a.group * (D / 8);  // of 16 bytes; the query heads of a token lie side by side
+    for (int t = from; t < to; ++t) {
+      const int64_t at = (int64_t)t * a.q_heads + head * a.group;
+      for (int i = threadIdx.x; i < pieces; i += blockDim.x)
+        store_any<u32x4>(a.out + at * (D * 2) + (int64_t)i * 16, u32x4{0u, 0u, 0u, 0u});
+      if (a.lse)
+        for (int i = threadIdx.x; i < a.group; i += blockDim.x) a.lse[at + i] = -INFINITY;
+    }
+  };
+  const int end = seq.q0 + seq.q_len;
+  const int from = b == 0 ? 0 : seq.q0, to = b == a.batch - 1 ? (int)a.total_q : end, held = min(end, seq.q0 + a.max_q);
+  if (__builtin_expect(mine & ((from != seq.q0) | (held != to)), 0)) {
+    clear(from, seq.q0);
+    clear(held, to);
+  }
+}
 
 // The run of keys of a work-group.  Consecutive work-groups go to the 8 dies in turn: unrotated, 4 or 8 runs would give
 // each die the same run of every sequence, and the later runs of short sequences are empty (64 sequences of 512 to
@@ -174,7 +199,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows16_kernel(AttnArgs a) {
   const int tile = blockIdx.x / a.splits, head = blockIdx.y, b = blockIdx.z;
   const int split = split_of(a, blockIdx.x % a.splits, head, b);
   const Seq seq(a, b);
-  const int rows = seq.q_len * a.group;
+  clear_unheld<D>(a, seq, head, b, blockIdx.x == 0 && a.splits == 1);
+  const int rows = seq.rows(a);
   if (tile * 16 >= rows) return;
   const int r = tile * 16 + n16;
   const bool real = r < rows;
@@ -526,7 +552,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(AttnArgs a) {
   const int tile = blockIdx.x / a.splits, head = blockIdx.y, b = blockIdx.z;
   const int split = split_of(a, blockIdx.x % a.splits, head, b);
   const Seq seq(a, b);
-  const int rows = seq.q_len * a.group, row0 = tile * kRows;
+  clear_unheld<D>(a, seq, head, b, blockIdx.x == 0 && a.splits == 1);
+  const int rows = seq.rows(a), row0 = tile * kRows;
   if (row0 >= rows) return;
   const int end_seen = seq.last_seen(a, (min(row0 + kRows, rows) - 1) / a.group) + 1;
   const int begin = (int)min((int64_t)split * a.split_len, (int64_t)0x7fffffff - 512);
@@ -550,6 +577,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(AttnArgs a) {
   const int wave_row = min(row0 + (wave + 1) * 32, rows) - 1;
   const int wave_end = row0 + wave * 32 < rows ? seq.last_seen(a, wave_row / a.group) + 1 : 0;
 
+  // (constant memory: behind the stores above the compiler would look pages up on the vector unit; 8 prompts of 2048:
+  // 466 -> 519 us)
+  const __attribute__((address_space(4))) int32_t* table =
+      (const __attribute__((address_space(4))) int32_t*)(a.table + b * a.width);
   // this wave brings 16 keys of each tile: a lane a quarter of one key, and an octet of four keys' values
   uint32_t kw[kKWords], ks, vw[kVWords], vs;
   bool ok = false;
@@ -557,7 +588,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tile_kernel(AttnArgs a) {
   auto fetch = [&](int pos) {
     const int p0 = pos + 16 * wave;
     int page = -1;
-    if (p0 < end) page = a.table[b * a.width + (p0 >> a.c.shift)];
+    if (p0 < end) page = table[p0 >> a.c.shift];
     page = __builtin_amdgcn_readfirstlane(page);
     ok = page >= 0 && page < a.c.pages;
     ks = 1u;
@@ -782,7 +813,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   __shared__ float red_l[16];
   const int head = blockIdx.y, b = blockIdx.z, r = blockIdx.x;
   const Seq seq(a, b);
-  if (r >= seq.q_len * a.group) return;
+  clear_unheld<D>(a, seq, head, b, r == 0);
+  if (r >= seq.rows(a)) return;
   const int t = r / a.group;
   const int64_t at = (int64_t)(seq.q0 + t) * a.q_heads + head * a.group + (r - t * a.group);
   // runs that hold a position this row sees
@@ -938,7 +970,9 @@ extern "C" int mpq_kv_attend(const void* q, int dtype, int64_t total_q, int64_t 
   MPQ_CHECK_ARG(table_width <= 0x7ffff000 / page && max_kv >= 0 && max_kv <= table_width * page,
                 "mpq_kv_attend: up to %lld positions, the table holds %lld pages of %d", (long long)max_kv,
                 (long long)table_width, page);
-  if (total_q == 0 || batch == 0 || max_q == 0) return kOk;
+  if (total_q == 0) return kOk;
+  MPQ_CHECK_ARG(batch >= 1 && max_q >= 1, "mpq_kv_attend: %lld tokens do not fit %lld sequences of up to %lld",
+                (long long)total_q, (long long)batch, (long long)max_q);
   MPQ_CHECK_ARG(q && kv_lens && q_starts && out && (block_table || table_width == 0), "mpq_kv_attend: null pointer");
   MPQ_CHECK_ARG(k_codes && k_scales && v_codes && v_scales, "mpq_kv_attend: null cache");
   const Plan p = plan_of(batch, heads, q_heads / heads, max_q, max_kv);
@@ -954,6 +988,8 @@ extern "C" int mpq_kv_attend(const void* q, int dtype, int64_t total_q, int64_t 
   a.total_q = total_q;
   a.q_heads = q_heads;
   a.group = q_heads / heads;
+  a.batch = (int)batch;
+  a.max_q = (int)max_q;
   a.table = block_table;
   a.width = table_width;
   a.kv_lens = kv_lens;

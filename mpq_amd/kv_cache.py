@@ -146,9 +146,10 @@ class QuantizedKVCache:
                out: Optional[torch.Tensor] = None, return_lse: bool = False):
         """Attention of the new tokens ``q`` (tokens, query heads, dim) over the cache that already holds them.
 
-        Sequence i is the tokens ``q_starts[i]`` to ``q_starts[i + 1]`` (batch + 1, int32; the last entry is the number
-        of tokens; no sequence has more than ``max_q``) over the positions below ``kv_lens[i]`` (batch, int32) of its
-        row of ``block_table``.  Query heads h * G to h * G + G - 1 read key/value head h.  With ``causal`` the last
+        Sequence i is the tokens ``q_starts[i]`` to ``q_starts[i + 1]`` (batch + 1, int32, in rising order; no sequence
+        has more than ``max_q``) over the positions below ``kv_lens[i]`` (batch, int32) of its row of
+        ``block_table``.  Tokens before the first sequence, behind the last one (a batch padded to a captured size) or
+        behind ``max_q`` of their sequence see nothing.  Query heads h * G to h * G + G - 1 read key/value head h.  With ``causal`` the last
         new token sees every position, the one before it all but the last, and so on.  ``scale`` defaults to
         ``dim ** -0.5``.  ``max_kv`` is the longest length if the caller knows it (default: what the table can
         hold); the work is split by it.  A row that sees nothing is 0.  With ``return_lse`` the logarithm

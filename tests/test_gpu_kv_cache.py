@@ -404,3 +404,63 @@ def test_read_nan_blocks(gpu, fmt, dtype):
         got, want = got.cpu(), om.values(x, fmt).to(dtype)
         assert int(want.isnan().sum()) == 64 and torch.equal(got.isnan(), want.isnan())
         assert torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,new,dim,group", [
+    ([40, 17], [1, 1], 64, 4),          # 16 rows, one run of keys
+    ([3000, 1500], [1, 2], 128, 7),     # 16 rows, runs joined
+    ([300, 200], [90, 40], 128, 2),     # 128 rows, one run
+    ([6000, 900], [60, 33], 64, 4),     # 128 rows, runs joined
+])
+def test_attend_tokens_outside_every_sequence_are_zero(gpu, dtype, lens, new, dim, group):
+    """Padding before and behind the sequences, and a sequence longer than max_q: 0 with lse -inf; every other token is bit
+    for bit what it is without them."""
+    b = _Batch(gpu, lens, 2, dim, 16, "mxfp8", dtype).fill()
+    n = sum(new)
+    table, kv = b.table.to(gpu), torch.tensor(lens, dtype=torch.int32, device=gpu)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=gpu)  # noqa: E731
+    q = torch.randn(n + 9, 2 * group, dim, generator=b.g).to(dtype).to(gpu)
+    starts, most = [4, 4 + new[0], 4 + n], max(new)
+    front = torch.cat([q[4: 4 + n], q[:9]])  # as many tokens: the same split of the work
+    want, lse = (t[:n] for t in b.cache.attend(front, table, kv, i32([0, new[0], n]), max(most, n + 9), return_lse=True))
+    out = torch.full_like(q, math.nan)
+    torch.full((n + 9, 2 * group), math.nan, device=gpu)  # what the memory of lse may hold
+    got, gl = b.cache.attend(q, table, kv, i32(starts), max(most, n + 9), out=out, return_lse=True)
+    none = torch.ones(n + 9, dtype=torch.bool)
+    none[4: 4 + n] = False
+    assert not bool(got[none].any()) and bool((gl[none] == -math.inf).all())
+    assert torch.equal(got[4: 4 + n], want) and torch.equal(gl[4: 4 + n], lse)
+
+
+@pytest.mark.parametrize("lens,new,max_q,group", [([50, 60], [5, 1], 3, 4), ([4000, 60], [5, 1], 3, 4),
+                                                  ([500, 300], [200, 5], 103, 2), ([6000, 300], [100, 5], 53, 2)])
+def test_attend_tokens_behind_max_q_are_zero(gpu, lens, new, max_q, group):
+    """A caller's max_q below a sequence's new tokens: those behind it are 0, the others are right."""
+    dim = 64
+    b = _Batch(gpu, lens, 1, dim, 16, "mxfp4", torch.bfloat16).fill()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=gpu)  # noqa: E731
+    n = sum(new)
+    q = torch.randn(n, group, dim, generator=b.g).to(torch.bfloat16).to(gpu)
+    args = (b.table.to(gpu), i32(lens), i32([0, new[0], n]))
+    got, lse = b.cache.attend(q, *args, max_q, out=torch.full_like(q, math.nan), return_lse=True)
+    want, wl = b.cache.attend(q, *args, max(new), return_lse=True)
+    held = torch.cat([torch.arange(m) < max_q for m in new])
+    assert not bool(got[~held].any()) and bool((lse[~held] == -math.inf).all())
+    assert torch.allclose(got[held].float(), want[held].float(), rtol=2 ** -6, atol=2 ** -8)
+    assert torch.allclose(lse[held], wl[held], rtol=1e-5, atol=1e-5)
+
+
+def test_attend_refuses_tokens_without_sequences(gpu):
+    """The C entry: tokens, but no sequence or none with a token."""
+    from mpq_amd import _lib
+
+    c = QuantizedKVCache(2, 16, 1, 64, device=gpu)
+    q = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device=gpu)
+    out, lens = torch.empty_like(q), torch.zeros(2, dtype=torch.int32, device=gpu)
+    for batch, max_q in ((0, 3), (1, 0)):
+        rc = _lib.load().mpq_kv_attend(q.data_ptr(), 1, 3, 128, 64, 2, batch, lens.data_ptr(), 1, lens.data_ptr(),
+                                       lens.data_ptr(), max_q, 16, *c._call, 0.125, 1, out.data_ptr(), None, None, 0,
+                                       _lib.stream_handle(gpu))
+        with pytest.raises(Exception, match="do not fit"):
+            _lib.check(rc, "mpq_kv_attend")
