@@ -22,13 +22,22 @@ from . import _lib, mx, ops
 HEAD_SIZES = (64, 128)
 
 
+def _over(cls, k_codes, k_scales, v_codes, v_scales, fmt, dtype) -> "QuantizedKVCache":
+    """A copied or unpickled cache, with the addresses of its own tensors."""
+    return cls.from_tensors(k_codes, k_scales, v_codes, v_scales, fmt=fmt, dtype=dtype)
+
+
 class QuantizedKVCache:
     """A pool of ``num_pages`` pages of ``page_size`` tokens (a power of two from 16).
 
     ``k_codes`` (pages, heads, page, bytes of a token's codes) and ``k_scales`` (pages, heads, page, dim / 32) hold the
     keys token by token; ``v_codes`` (pages, heads, page / 4, dim / 8, 4, bytes of 8 codes) and ``v_scales``
     (pages, heads, page / 4, dim / 32, 4) the values in groups of four tokens, all uint8.  ``dtype`` (bfloat16 or
-    float16) is the type of the keys, values and queries."""
+    float16) is the type of the keys, values and queries.  A cache keeps these for life (their contents may change):
+    the calls hold their addresses."""
+
+    _FIXED = frozenset(("k_codes", "k_scales", "v_codes", "v_scales", "fmt", "dtype", "device", "num_pages", "heads",
+                        "page_size", "head_dim", "_f", "_call"))
 
     def __init__(self, num_pages: int, page_size: int, heads: int, head_dim: int, *, fmt: str = "mxfp8",
                  dtype: torch.dtype = torch.bfloat16, device: Union[str, torch.device] = "cuda") -> None:
@@ -58,14 +67,27 @@ class QuantizedKVCache:
         self._set(k_codes, k_scales, v_codes, v_scales, fmt, dtype)
         return self
 
+    def __setattr__(self, name: str, value) -> None:
+        if name in self._FIXED:
+            raise AttributeError(f"{name} of a cache is fixed; QuantizedKVCache.from_tensors makes one over other tensors")
+        super().__setattr__(name, value)
+
+    def __delattr__(self, name: str) -> None:
+        if name in self._FIXED:
+            raise AttributeError(f"{name} of a cache is fixed")
+        super().__delattr__(name)
+
+    def __reduce__(self):
+        return _over, (type(self), self.k_codes, self.k_scales, self.v_codes, self.v_scales, self.fmt, self.dtype)
+
     def _set(self, k_codes, k_scales, v_codes, v_scales, fmt, dtype) -> None:
-        self._f = mx._fmt(fmt)
+        f = mx._fmt(fmt)
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"dtype must be bfloat16 or float16, got {dtype}")
         if k_codes.dim() != 4:
             raise ValueError(f"k_codes must be (pages, heads, page, bytes), got {tuple(k_codes.shape)}")
         N, H, P, width = k_codes.shape
-        wide = 2 if self._f == 0 else 1
+        wide = 2 if f == 0 else 1
         D = width * wide
         if N < 1 or H < 1 or P < 16 or P > 65536 or P & (P - 1) or D not in HEAD_SIZES:
             raise ValueError(f"k_codes {tuple(k_codes.shape)} are no {fmt} cache: pages of a power of two from 16 "
@@ -78,11 +100,9 @@ class QuantizedKVCache:
             if t.shape != shapes[i] or t.dtype != torch.uint8 or not t.is_contiguous() or at[i] % 16:
                 raise ValueError(f"{('k_codes', 'k_scales', 'v_codes', 'v_scales')[i]} must be a contiguous, 16-byte "
                                  f"aligned uint8 tensor of shape {shapes[i]}, got {t.dtype} {tuple(t.shape)}")
-        self.device = mx._on_device(*tensors)
-        self.k_codes, self.k_scales, self.v_codes, self.v_scales = tensors
-        self.fmt, self.dtype = fmt, dtype
-        self.num_pages, self.heads, self.page_size, self.head_dim = N, H, P, D
-        self._call = (self._f, H, D, P, N, *at)
+        self.__dict__.update(device=mx._on_device(*tensors), k_codes=k_codes, k_scales=k_scales, v_codes=v_codes,
+                             v_scales=v_scales, fmt=fmt, dtype=dtype, num_pages=N, heads=H, page_size=P, head_dim=D,
+                             _f=f, _call=(f, H, D, P, N, *at))
 
     def _tokens(self, t: torch.Tensor, name: str, heads: Optional[int] = None) -> torch.Tensor:
         """(tokens, heads, dim) with a contiguous last dimension."""
