@@ -14,6 +14,7 @@ Tensors live on the ROCm device; there is no CPU path, and no gradient.
 from __future__ import annotations
 
 import math
+import operator
 from typing import Optional, Tuple, Union
 
 import torch
@@ -63,9 +64,12 @@ class MXTensor:
     """A quantised tensor: ``codes`` (rows, :func:`code_bytes`) and ``scales`` (rows, padded cols / 32), both uint8.
 
     ``cols`` is the length of the last dimension; ``lead`` the other ones (``rows`` is their product).  In ``mxfp4``
-    a byte holds two codes, the first in its low half.  Codes behind ``cols`` are zero."""
+    a byte holds two codes, the first in its low half.  Codes behind ``cols`` are zero.  The attributes are checked
+    once and cannot be replaced (their contents may change)."""
 
-    __slots__ = ("codes", "scales", "cols", "fmt", "lead", "rows", "device", "_f")
+    __slots__ = ("_codes", "_scales", "_cols", "_fmt", "_lead", "_rows", "_device", "_f")
+    codes, scales, cols, fmt, lead, rows, device = (
+        property(operator.attrgetter("_" + n)) for n in ("codes", "scales", "cols", "fmt", "lead", "rows", "device"))
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int, fmt: str = "mxfp4",
                  lead: Optional[Tuple[int, ...]] = None) -> None:
@@ -87,13 +91,13 @@ class MXTensor:
         self._set(codes, scales, cols, fmt, f, lead, rows, _on_device(codes, scales))
 
     def _set(self, codes, scales, cols, fmt, f, lead, rows, device) -> "MXTensor":
-        self.codes, self.scales, self.cols, self.fmt, self._f = codes, scales, cols, fmt, f
-        self.lead, self.rows, self.device = lead, rows, device
+        self._codes, self._scales, self._cols, self._fmt, self._f = codes, scales, cols, fmt, f
+        self._lead, self._rows, self._device = lead, rows, device
         return self
 
     @property
     def shape(self) -> Tuple[int, ...]:
-        return (*self.lead, self.cols)
+        return (*self._lead, self._cols)
 
 
 def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
@@ -129,12 +133,12 @@ def quantize(x: torch.Tensor, fmt: str = "mxfp4") -> MXTensor:
 
 def dequantize(t: MXTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values that ``t`` stands for (exact in float32 and bfloat16)."""
-    dt, dev = _dtype(dtype, "dtype"), t.device
+    dt, dev = _dtype(dtype, "dtype"), t._device
     out = torch.empty(t.shape, dtype=dtype, device=dev)
-    if t.rows:
+    if t._rows:
         with ops.on_device(dev):
-            _lib.check(_lib.load().mpq_mx_dequantize(t.codes.data_ptr(), t.scales.data_ptr(), t.rows, t.cols, t._f,
-                                                     out.data_ptr(), dt, t.cols, _lib.stream_handle(dev)),
+            _lib.check(_lib.load().mpq_mx_dequantize(t._codes.data_ptr(), t._scales.data_ptr(), t._rows, t._cols, t._f,
+                                                     out.data_ptr(), dt, t._cols, _lib.stream_handle(dev)),
                        "mpq_mx_dequantize")
     return out
 
@@ -150,14 +154,14 @@ def linear(x: Union[torch.Tensor, MXTensor], weight: MXTensor, bias: Optional[to
 
     Sums are held in fp32.  With ``mxfp8`` the matrix core cuts the terms of each 32-value block at 2^-13 of the
     block's largest product, some 1e-4 of the result: fine for 16-bit results, and less than the format's own error."""
-    if weight._f != 0 or len(weight.lead) != 1:
+    if weight._f != 0 or len(weight._lead) != 1:
         raise ValueError("weight must be a 2-D mxfp4 MXTensor (out features x in features)")
     given = isinstance(x, MXTensor)
     f = x._f if given else _fmt(act_format)
-    shape, rows, cols = x.shape, weight.rows, weight.cols
+    shape, rows, cols = x.shape, weight._rows, weight._cols
     if len(shape) < 1 or shape[-1] != cols:
         raise ValueError(f"x has shape {tuple(shape)}, weight takes {cols} features")
-    dev = _on_device(weight.codes, x.codes if given else x, bias, out)
+    dev = _on_device(weight._codes, x._codes if given else x, bias, out)
     if dtype is None:
         dtype = out.dtype if out is not None else torch.bfloat16 if given else x.dtype
     odt = _dtype(dtype, "dtype")
@@ -176,14 +180,14 @@ def linear(x: Union[torch.Tensor, MXTensor], weight: MXTensor, bias: Optional[to
         return out
     lib = _lib.load()
     if given:
-        src = (None, 0, cols, x.codes.data_ptr(), x.scales.data_ptr())
+        src = (None, 0, cols, x._codes.data_ptr(), x._scales.data_ptr())
     else:
         x, ld = _rows(x)
         src = (x.data_ptr(), xdt, ld, None, None)
     need = lib.mpq_mx_linear_workspace_size(tokens, cols, rows, f)
     ws = ops.workspace(need, dev) if need else None
     with ops.on_device(dev):
-        _lib.check(lib.mpq_mx_linear(*src, f, tokens, cols, weight.codes.data_ptr(), weight.scales.data_ptr(), rows,
+        _lib.check(lib.mpq_mx_linear(*src, f, tokens, cols, weight._codes.data_ptr(), weight._scales.data_ptr(), rows,
                                      None if bias is None else bias.data_ptr(), out.data_ptr(), odt, rows,
                                      None if ws is None else ws.data_ptr(), need, _lib.stream_handle(dev)),
                    "mpq_mx_linear")

@@ -42,3 +42,17 @@ def test_a_copied_cache_addresses_its_own_tensors(on_cpu, way):
     assert d._call == (*c._call[:5], *(t.data_ptr() for t in tensors))
     assert (d.fmt, d.dtype, d.num_pages, d.heads, d.page_size, d.head_dim) == ("mxfp8", torch.float16, 3, 2, 16, 64)
     assert (d.k_codes is c.k_codes) == (way is copy.copy)
+
+
+def test_a_quantised_tensor_keeps_what_was_checked(on_cpu):
+    """The kernels go by the sizes that the constructor checked against the tensors."""
+    t = mx.MXTensor(torch.zeros(6, 128, dtype=torch.uint8), torch.ones(6, 8, dtype=torch.uint8), 200, lead=(2, 3))
+    for name, value in (("codes", t.codes[:2]), ("scales", t.scales[:2]), ("rows", 7), ("cols", 900), ("fmt", "mxfp8"),
+                        ("lead", (6,)), ("device", None), ("shape", (6, 200))):
+        with pytest.raises(AttributeError):
+            setattr(t, name, value)
+        with pytest.raises(AttributeError):
+            delattr(t, name)
+    for u in (t, copy.copy(t), copy.deepcopy(t), pickle.loads(pickle.dumps(t))):
+        assert (u.shape, u.rows, u.cols, u.lead, u.fmt) == ((2, 3, 200), 6, 200, (2, 3), "mxfp4")
+        assert torch.equal(u.codes, t.codes) and torch.equal(u.scales, t.scales) and u.device == t.device
