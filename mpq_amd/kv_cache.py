@@ -139,7 +139,7 @@ class QuantizedKVCache:
             vt, vh, _ = v.stride()
             with ops.on_device(dev):
                 _lib.check(_lib.load().mpq_kv_write(k.data_ptr(), v.data_ptr(), mx.DTYPES[self.dtype], n, kt, kh, vt, vh,
-                                                    slots.data_ptr(), *self._call, _lib.stream_handle(dev)),
+                                                    slots.data_ptr(), *self._call, ops.raw_stream(dev)),
                            "mpq_kv_write")
 
     def read(self, block_table: torch.Tensor, starts: torch.Tensor, total: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -158,7 +158,7 @@ class QuantizedKVCache:
             with ops.on_device(dev):
                 _lib.check(_lib.load().mpq_kv_read(block_table.data_ptr(), B, W, starts.data_ptr(), total, *self._call,
                                                    k.data_ptr(), v.data_ptr(), mx.DTYPES[self.dtype],
-                                                   _lib.stream_handle(dev)), "mpq_kv_read")
+                                                   ops.raw_stream(dev)), "mpq_kv_read")
         return k, v
 
     def attend(self, q: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, q_starts: torch.Tensor,
@@ -167,13 +167,14 @@ class QuantizedKVCache:
         """Attention of the new tokens ``q`` (tokens, query heads, dim) over the cache that already holds them.
 
         Sequence i is the tokens ``q_starts[i]`` to ``q_starts[i + 1]`` (batch + 1, int32, in rising order; no sequence
-        has more than ``max_q``) over the positions below ``kv_lens[i]`` (batch, int32) of its row of
-        ``block_table``.  Tokens before the first sequence, behind the last one (a batch padded to a captured size) or
-        behind ``max_q`` of their sequence see nothing.  Query heads h * G to h * G + G - 1 read key/value head h.  With ``causal`` the last
-        new token sees every position, the one before it all but the last, and so on.  ``scale`` defaults to
-        ``dim ** -0.5``.  ``max_kv`` is the longest length if the caller knows it (default: what the table can
-        hold); the work is split by it.  A row that sees nothing is 0.  With ``return_lse`` the logarithm
-        of each row's sum of exponentials (tokens, query heads; float32) comes too."""
+        has more than ``max_q``) over the positions below ``kv_lens[i]`` (batch, int32) of its row of ``block_table``.
+        Tokens before the first sequence, behind the last one (a batch padded to a captured size) or behind ``max_q``
+        of their sequence see nothing. Query heads h * G to h * G + G - 1 read key/value head h. With ``causal`` the
+        last new token sees every position, the one before it all but the last, and so on. ``scale`` defaults to ``dim
+        ** -0.5``. ``max_kv`` is the longest length if the caller knows it (default: what the table can hold); the work
+        is split by it. A row that sees nothing is 0. With ``return_lse`` the logarithm of each row's sum of
+        exponentials (tokens, query heads; float32) comes too. A backward pass through the results raises (a given
+        ``out`` is left out of it)."""
         q = self._tokens(q, "q")
         block_table = self._table(block_table)
         B, W = block_table.shape
@@ -189,7 +190,8 @@ class QuantizedKVCache:
         if max_kv < 0 or max_kv > most:
             raise ValueError(f"max_kv must be between 0 and the table's {most} positions, got {max_kv}")
         dev = mx._on_device(self.k_codes, q, block_table, kv_lens, q_starts, out)
-        if out is None:
+        fresh = out is None
+        if fresh:
             out = torch.empty((T, Hq, D), dtype=self.dtype, device=dev)
         elif out.shape != q.shape or out.dtype != self.dtype or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {self.dtype} tensor of shape {(T, Hq, D)}")
@@ -206,6 +208,9 @@ class QuantizedKVCache:
                                              max_kv, *self._call, D ** -0.5 if scale is None else float(scale),
                                              1 if causal else 0, out.data_ptr(),
                                              None if lse is None else lse.data_ptr(),
-                                             None if ws is None else ws.data_ptr(), need, _lib.stream_handle(dev)),
+                                             None if ws is None else ws.data_ptr(), need, ops.raw_stream(dev)),
                            "mpq_kv_attend")
+        if q.requires_grad:
+            out = mx._no_gradient("QuantizedKVCache.attend", out, q) if fresh else out
+            lse = mx._no_gradient("QuantizedKVCache.attend", lse, q) if return_lse else None
         return (out, lse) if return_lse else out

@@ -9,7 +9,7 @@ A block is 32 consecutive values of the last dimension with one power-of-two sca
 Values are rounded to nearest, ties to even, and saturate.  A block with a NaN or an infinity reads back as NaN.
 No counterpart in the reference, whose formats are integer grids and the E8P12 codebook.
 
-Tensors live on the ROCm device; there is no CPU path, and no gradient.
+Tensors live on the ROCm device; there is no CPU path, and no gradient: a backward pass through a result raises.
 """
 from __future__ import annotations
 
@@ -58,6 +58,26 @@ def _on_device(*ts: Optional[torch.Tensor]) -> torch.device:
         if t is not None and t.device != dev:
             raise ValueError("all tensors must be on the same device")
     return dev
+
+
+class _NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, name, out, x, bias):
+        ctx.name = name
+        ctx.mark_dirty(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name} has no gradient")
+
+
+def _no_gradient(name: str, out: torch.Tensor, x: Optional[torch.Tensor],
+                 bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``out``, through which a backward pass raises if gradients of ``x`` or ``bias`` are recorded."""
+    if (x is not None and x.requires_grad or bias is not None and bias.requires_grad) and torch.is_grad_enabled():
+        return _NoGradient.apply(name, out, x, bias)
+    return out
 
 
 class MXTensor:
@@ -127,7 +147,7 @@ def quantize(x: torch.Tensor, fmt: str = "mxfp4") -> MXTensor:
         x, ld = _rows(x)
         with ops.on_device(dev):
             _lib.check(_lib.load().mpq_mx_quantize(x.data_ptr(), dt, rows, cols, ld, f, codes.data_ptr(),
-                                                   scales.data_ptr(), _lib.stream_handle(dev)), "mpq_mx_quantize")
+                                                   scales.data_ptr(), ops.raw_stream(dev)), "mpq_mx_quantize")
     return MXTensor.__new__(MXTensor)._set(codes, scales, cols, fmt, f, tuple(shape[:-1]), rows, dev)
 
 
@@ -138,7 +158,7 @@ def dequantize(t: MXTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     if t._rows:
         with ops.on_device(dev):
             _lib.check(_lib.load().mpq_mx_dequantize(t._codes.data_ptr(), t._scales.data_ptr(), t._rows, t._cols, t._f,
-                                                     out.data_ptr(), dt, t._cols, _lib.stream_handle(dev)),
+                                                     out.data_ptr(), dt, t._cols, ops.raw_stream(dev)),
                        "mpq_mx_dequantize")
     return out
 
@@ -152,11 +172,13 @@ def linear(x: Union[torch.Tensor, MXTensor], weight: MXTensor, bias: Optional[to
     comes as an :class:`MXTensor` in either format.  The result has ``dtype`` (default: that of ``x``; bfloat16 for an
     :class:`MXTensor`); ``out`` (contiguous, of that shape and type) receives it in place of a new tensor.
 
+    A backward pass through the result raises (a given ``out`` is left out of it).
+
     Sums are held in fp32.  With ``mxfp8`` the matrix core cuts the terms of each 32-value block at 2^-13 of the
     block's largest product, some 1e-4 of the result: fine for 16-bit results, and less than the format's own error."""
     if weight._f != 0 or len(weight._lead) != 1:
         raise ValueError("weight must be a 2-D mxfp4 MXTensor (out features x in features)")
-    given = isinstance(x, MXTensor)
+    given, fresh = isinstance(x, MXTensor), out is None
     f = x._f if given else _fmt(act_format)
     shape, rows, cols = x.shape, weight._rows, weight._cols
     if len(shape) < 1 or shape[-1] != cols:
@@ -189,6 +211,8 @@ def linear(x: Union[torch.Tensor, MXTensor], weight: MXTensor, bias: Optional[to
     with ops.on_device(dev):
         _lib.check(lib.mpq_mx_linear(*src, f, tokens, cols, weight._codes.data_ptr(), weight._scales.data_ptr(), rows,
                                      None if bias is None else bias.data_ptr(), out.data_ptr(), odt, rows,
-                                     None if ws is None else ws.data_ptr(), need, _lib.stream_handle(dev)),
+                                     None if ws is None else ws.data_ptr(), need, ops.raw_stream(dev)),
                    "mpq_mx_linear")
+    if fresh and (bias is not None or not given and x.requires_grad):
+        return _no_gradient("mx.linear", out, None if given else x, bias)
     return out

@@ -49,6 +49,11 @@ def on_device(dev: torch.device):
     return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
+def raw_stream(dev: torch.device) -> int:
+    """Handle of the current stream of a tensor's device (a ROCm device with its number)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
 

@@ -464,3 +464,13 @@ def test_attend_refuses_tokens_without_sequences(gpu):
                                        _lib.stream_handle(gpu))
         with pytest.raises(Exception, match="do not fit"):
             _lib.check(rc, "mpq_kv_attend")
+
+
+def test_attend_backward_raises(gpu):
+    b = _Batch(gpu, [40], 1, 64, 16, "mxfp8", torch.bfloat16).fill()
+    q, _, want = b.attend([3], 2)
+    for which in (0, 1):
+        _, _, got = b.attend([3], 2, q=q.clone().requires_grad_(), return_lse=True)
+        assert torch.equal(got[0], want)
+        with pytest.raises(RuntimeError, match="attend has no gradient"):
+            got[which].float().sum().backward()

@@ -56,3 +56,18 @@ def test_a_quantised_tensor_keeps_what_was_checked(on_cpu):
     for u in (t, copy.copy(t), copy.deepcopy(t), pickle.loads(pickle.dumps(t))):
         assert (u.shape, u.rows, u.cols, u.lead, u.fmt) == ((2, 3, 200), 6, 200, (2, 3), "mxfp4")
         assert torch.equal(u.codes, t.codes) and torch.equal(u.scales, t.scales) and u.device == t.device
+
+
+def test_a_backward_pass_raises():
+    """Results hold no gradient: where one would be recorded, its backward pass says so instead of leaving it out."""
+    x, bias = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+    for inputs in ((x,), (None, bias), (x, bias)):
+        out = torch.zeros(3)
+        got = mx._no_gradient("op", out, *inputs)
+        assert got.requires_grad and got.data_ptr() == out.data_ptr()
+        with pytest.raises(RuntimeError, match="op has no gradient"):
+            (got * 2 + x).sum().backward()
+    out = torch.zeros(3)
+    assert mx._no_gradient("op", out, x.detach(), None) is out and mx._no_gradient("op", out, None) is out
+    with torch.no_grad():
+        assert mx._no_gradient("op", out, x) is out and not out.requires_grad
