@@ -187,6 +187,10 @@ __device__ __forceinline__ u32x4 mx_decode8(u32x2 w, float s) {
 hipError_t mx_quantize_rows(const void* x, int type, int64_t rows, int64_t cols, int64_t ld, int fmt, uint8_t* codes,
                             uint8_t* scales, hipStream_t stream);
 
+// Threads of one launch of the kernels that go over any number of rows: a launch whose threads along x pass 2^32 is cut to
+// the rest without an error, so longer calls are several launches.
+constexpr int64_t kMxLaunch = (int64_t)1 << 31;
+
 __host__ __device__ inline int64_t mx_padded(int64_t cols) { return (cols + kMxRow - 1) / kMxRow * kMxRow; }
 __host__ __device__ inline int64_t mx_code_bytes(int64_t padded, int fmt) { return fmt == kMxFp4 ? padded / 2 : padded; }
 

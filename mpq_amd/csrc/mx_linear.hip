@@ -589,10 +589,16 @@ hipError_t launch_few(const Args& a) {
   const int lds = FUSED ? (int)std::max<int64_t>(red, fused_bytes(a.tokens, a.padded, XF)) : red;
   auto kernel = few_kernel<XF, FUSED, XTYPE, OTYPE>;
   if (hipError_t e = allow_lds(kernel, lds); e != hipSuccess) return e;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)mpq_cdiv(a.rows, 16)), dim3(64 * kFewWaves), lds, a.stream,
-                     static_cast<const char*>(a.x), a.ldx, a.xc, a.xs, (int)a.tokens, a.cols, a.padded, a.wc, a.ws,
-                     a.rows, a.bias, a.out, a.ldo);
-  return hipGetLastError();
+  constexpr int64_t most = kMxLaunch / (64 * kFewWaves) * 16;
+  for (int64_t f = 0; f < a.rows; f += most) {
+    const int64_t n = std::min(most, a.rows - f);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)mpq_cdiv(n, 16)), dim3(64 * kFewWaves), lds, a.stream,
+                       static_cast<const char*>(a.x), a.ldx, a.xc, a.xs, (int)a.tokens, a.cols, a.padded,
+                       a.wc + f * (a.padded / 2), a.ws + f * (a.padded / kMxBlock), n, a.bias ? a.bias + f : nullptr,
+                       static_cast<char*>(a.out) + f * (OTYPE == kMxF32 ? 4 : 2), a.ldo);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <int XF, int FA, int TB, int WT, int OTYPE>
@@ -692,8 +698,9 @@ extern "C" int mpq_mx_linear(const void* x, int dtype, int64_t ldx, const uint8_
   const bool given = x_codes != nullptr;
   MPQ_CHECK_ARG(given ? x_scales != nullptr : (x != nullptr && ldx >= cols), "mpq_mx_linear: no tokens given");
   MPQ_CHECK_ARG(w_codes && w_scales && out && ldo >= rows, "mpq_mx_linear: null pointer or short output rows");
+  // (the tiles of a launch of 512 threads each: more results than the card holds)
   MPQ_CHECK_ARG(cols <= (1 << 23) && tokens <= (1 << 30) && rows <= (1 << 30) &&
-                    mpq_cdiv(tokens, 64) * mpq_cdiv(rows, 64) <= 0x7ffffff0,
+                    mpq_cdiv(tokens, 256) * mpq_cdiv(rows, 256) <= (1 << 23) - 256,
                 "mpq_mx_linear: extent too large");
   const int64_t padded = mx_padded(cols);
   Args a = {x, dtype, ldx, x_codes, x_scales, tokens, cols, padded, w_codes, w_scales, rows, bias, out, ldo, nullptr,

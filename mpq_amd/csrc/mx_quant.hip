@@ -1,4 +1,6 @@
 // Quantisation of matrices into microscaled blocks and back (gfx950).
+#include <algorithm>
+
 #include "mx.h"
 
 namespace mpq {
@@ -122,25 +124,26 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* __restri
 struct Shape {
   int unroll;
   uint32_t pieces;
-  unsigned blocks;
+  int64_t most;  // rows of a launch
+  unsigned blocks(int64_t rows) const { return (unsigned)((rows * pieces + 3) / 4); }
 };
 
-bool shape_of(int64_t rows, int64_t padded, Shape* s) {
-  s->unroll = rows * padded >= (int64_t)512 * 4 * 4096 ? 4 : 1;
-  s->pieces = (uint32_t)((padded + 512 * s->unroll - 1) / (512 * s->unroll));
-  const int64_t blocks = (rows * s->pieces + 3) / 4;
-  s->blocks = (unsigned)blocks;
-  return blocks <= 0x7fffffff;
+Shape shape_of(int64_t rows, int64_t padded) {
+  Shape s;
+  s.unroll = rows * padded >= (int64_t)512 * 4 * 4096 ? 4 : 1;
+  s.pieces = (uint32_t)((padded + 512 * s.unroll - 1) / (512 * s.unroll));
+  s.most = kMxLaunch / 64 / s.pieces;
+  return s;
 }
 
 template <int TYPE, int FMT>
 void launch_quantize(const Shape& s, const void* x, int64_t rows, int64_t cols, int64_t ld, int64_t padded,
                      uint8_t* codes, uint8_t* scales, hipStream_t stream) {
   if (s.unroll == 4)
-    hipLaunchKernelGGL((quantize_kernel<TYPE, FMT, 4>), dim3(s.blocks), dim3(256), 0, stream,
+    hipLaunchKernelGGL((quantize_kernel<TYPE, FMT, 4>), dim3(s.blocks(rows)), dim3(256), 0, stream,
                        static_cast<const char*>(x), rows, cols, ld, padded, s.pieces, codes, scales);
   else
-    hipLaunchKernelGGL((quantize_kernel<TYPE, FMT, 1>), dim3(s.blocks), dim3(256), 0, stream,
+    hipLaunchKernelGGL((quantize_kernel<TYPE, FMT, 1>), dim3(s.blocks(rows)), dim3(256), 0, stream,
                        static_cast<const char*>(x), rows, cols, ld, padded, s.pieces, codes, scales);
 }
 
@@ -148,10 +151,10 @@ template <int TYPE, int FMT>
 void launch_dequantize(const Shape& s, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols,
                        int64_t padded, void* out, int64_t ld, hipStream_t stream) {
   if (s.unroll == 4)
-    hipLaunchKernelGGL((dequantize_kernel<TYPE, FMT, 4>), dim3(s.blocks), dim3(256), 0, stream, codes, scales, rows,
+    hipLaunchKernelGGL((dequantize_kernel<TYPE, FMT, 4>), dim3(s.blocks(rows)), dim3(256), 0, stream, codes, scales, rows,
                        cols, padded, s.pieces, static_cast<char*>(out), ld);
   else
-    hipLaunchKernelGGL((dequantize_kernel<TYPE, FMT, 1>), dim3(s.blocks), dim3(256), 0, stream, codes, scales, rows,
+    hipLaunchKernelGGL((dequantize_kernel<TYPE, FMT, 1>), dim3(s.blocks(rows)), dim3(256), 0, stream, codes, scales, rows,
                        cols, padded, s.pieces, static_cast<char*>(out), ld);
 }
 
@@ -160,20 +163,25 @@ void launch_dequantize(const Shape& s, const uint8_t* codes, const uint8_t* scal
 hipError_t mx_quantize_rows(const void* x, int type, int64_t rows, int64_t cols, int64_t ld, int fmt, uint8_t* codes,
                             uint8_t* scales, hipStream_t stream) {
   const int64_t padded = mx_padded(cols);
-  Shape s;
-  if (!shape_of(rows, padded, &s)) return hipErrorInvalidValue;
-#define MPQ_Q(T, F) launch_quantize<T, F>(s, x, rows, cols, ld, padded, codes, scales, stream)
-  if (fmt == kMxFp4) {
-    if (type == kMxF32) MPQ_Q(kMxF32, kMxFp4);
-    else if (type == kMxBf16) MPQ_Q(kMxBf16, kMxFp4);
-    else MPQ_Q(kMxF16, kMxFp4);
-  } else {
-    if (type == kMxF32) MPQ_Q(kMxF32, kMxFp8);
-    else if (type == kMxBf16) MPQ_Q(kMxBf16, kMxFp8);
-    else MPQ_Q(kMxF16, kMxFp8);
-  }
+  const Shape s = shape_of(rows, padded);
+  for (int64_t r = 0; r < rows; r += s.most) {
+    const int64_t n = std::min(s.most, rows - r);
+    const char* from = static_cast<const char*>(x) + r * ld * (type == kMxF32 ? 4 : 2);
+    uint8_t *c = codes + r * mx_code_bytes(padded, fmt), *b = scales + r * (padded / kMxBlock);
+#define MPQ_Q(T, F) launch_quantize<T, F>(s, from, n, cols, ld, padded, c, b, stream)
+    if (fmt == kMxFp4) {
+      if (type == kMxF32) MPQ_Q(kMxF32, kMxFp4);
+      else if (type == kMxBf16) MPQ_Q(kMxBf16, kMxFp4);
+      else MPQ_Q(kMxF16, kMxFp4);
+    } else {
+      if (type == kMxF32) MPQ_Q(kMxF32, kMxFp8);
+      else if (type == kMxBf16) MPQ_Q(kMxBf16, kMxFp8);
+      else MPQ_Q(kMxF16, kMxFp8);
+    }
 #undef MPQ_Q
-  return hipGetLastError();
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace mpq
@@ -205,19 +213,23 @@ extern "C" int mpq_mx_dequantize(const uint8_t* codes, const uint8_t* scales, in
   MPQ_CHECK_ARG(cols <= ((int64_t)1 << 31) && rows <= ((int64_t)1 << 40) / mx_padded(cols),
                 "mpq_mx_dequantize: extent too large");
   const int64_t padded = mx_padded(cols);
-  Shape s;
-  MPQ_CHECK_ARG(shape_of(rows, padded, &s), "mpq_mx_dequantize: extent too large");
-#define MPQ_D(T, F) launch_dequantize<T, F>(s, codes, scales, rows, cols, padded, out, ld, stream)
-  if (fmt == kMxFp4) {
-    if (dtype == kMxF32) MPQ_D(kMxF32, kMxFp4);
-    else if (dtype == kMxBf16) MPQ_D(kMxBf16, kMxFp4);
-    else MPQ_D(kMxF16, kMxFp4);
-  } else {
-    if (dtype == kMxF32) MPQ_D(kMxF32, kMxFp8);
-    else if (dtype == kMxBf16) MPQ_D(kMxBf16, kMxFp8);
-    else MPQ_D(kMxF16, kMxFp8);
-  }
+  const Shape s = shape_of(rows, padded);
+  for (int64_t r = 0; r < rows; r += s.most) {
+    const int64_t n = std::min(s.most, rows - r);
+    const uint8_t *c = codes + r * mx_code_bytes(padded, fmt), *b = scales + r * (padded / kMxBlock);
+    char* to = static_cast<char*>(out) + r * ld * (dtype == kMxF32 ? 4 : 2);
+#define MPQ_D(T, F) launch_dequantize<T, F>(s, c, b, n, cols, padded, to, ld, stream)
+    if (fmt == kMxFp4) {
+      if (dtype == kMxF32) MPQ_D(kMxF32, kMxFp4);
+      else if (dtype == kMxBf16) MPQ_D(kMxBf16, kMxFp4);
+      else MPQ_D(kMxF16, kMxFp4);
+    } else {
+      if (dtype == kMxF32) MPQ_D(kMxF32, kMxFp8);
+      else if (dtype == kMxBf16) MPQ_D(kMxBf16, kMxFp8);
+      else MPQ_D(kMxF16, kMxFp8);
+    }
 #undef MPQ_D
-  MPQ_LAUNCH_CHECK();
+    MPQ_LAUNCH_CHECK();
+  }
   return kOk;
 }

@@ -170,8 +170,8 @@ class QuantizedKVCache:
         has more than ``max_q``) over the positions below ``kv_lens[i]`` (batch, int32) of its row of ``block_table``.
         Tokens before the first sequence, behind the last one (a batch padded to a captured size) or behind ``max_q``
         of their sequence see nothing. Query heads h * G to h * G + G - 1 read key/value head h. With ``causal`` the
-        last new token sees every position, the one before it all but the last, and so on. ``scale`` defaults to ``dim
-        ** -0.5``. ``max_kv`` is the longest length if the caller knows it (default: what the table can hold); the work
+        last new token sees every position, the one before it all but the last, and so on. ``scale`` defaults to
+        ``dim ** -0.5``. ``max_kv`` is the longest length if the caller knows it (default: what the table can hold); the work
         is split by it. A row that sees nothing is 0. With ``return_lse`` the logarithm of each row's sum of
         exponentials (tokens, query heads; float32) comes too. A backward pass through the results raises (a given
         ``out`` is left out of it)."""

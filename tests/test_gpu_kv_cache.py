@@ -474,3 +474,47 @@ def test_attend_backward_raises(gpu):
         assert torch.equal(got[0], want)
         with pytest.raises(RuntimeError, match="attend has no gradient"):
             got[which].float().sum().backward()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+def test_write_more_tokens_than_a_launch_has_threads(gpu, fmt):
+    """A lane an octet: 2^19 tokens of 1024 heads of 64 are 2^32 threads, more than one launch takes."""
+    H, n = 1024, (1 << 19) + 9
+    cache = QuantizedKVCache(2, 16, H, 64, fmt=fmt, device=gpu)
+    at = [0, (1 << 18) - 1, 1 << 18, (1 << 19) - 1, 1 << 19, n - 1]
+    slots = torch.full((n,), -1, dtype=torch.int64, device=gpu)
+    slots[torch.tensor(at, device=gpu)] = torch.arange(6, device=gpu)
+    g = torch.Generator().manual_seed(3)
+    base = torch.randn(n + 64 * 8, generator=g).to(torch.bfloat16)  # a token's rows start one value after its predecessor's
+    k = base.to(gpu).as_strided((n, H, 64), (1, 0, 1))
+    cache.write(k, k, slots)
+    table = torch.tensor([[0]], dtype=torch.int32, device=gpu)
+    got = cache.read(table, torch.tensor([0, 6], dtype=torch.int32, device=gpu), 6)
+    want = torch.stack([om.values(base[i: i + 64], fmt) for i in at]).to(torch.bfloat16).unsqueeze(1).expand(6, H, 64)
+    for t in got:
+        assert torch.equal(t.cpu(), want)
+
+
+def test_read_more_tokens_than_a_launch_has_threads(gpu):
+    """As above, 64 GiB of keys and as many of values."""
+    H, n = 1024, (1 << 19) + 9
+    torch.cuda.empty_cache()
+    cache = QuantizedKVCache(3, 16, H, 64, device=gpu)
+    g = torch.Generator().manual_seed(3)
+    k = torch.randn(48, H, 64, generator=g).to(torch.bfloat16)
+    cache.write(k.to(gpu), -k.to(gpu), torch.arange(48, device=gpu))
+    table = torch.full((1, n // 16 + 1), -1, dtype=torch.int32, device=gpu)
+    pages = {0: 2, (1 << 18) // 16 - 1: 0, (1 << 18) // 16: 1, (1 << 19) // 16 - 1: 2, (1 << 19) // 16: 0}
+    for at, page in pages.items():
+        table[0, at] = page
+    got = cache.read(table, torch.tensor([0, n], dtype=torch.int32, device=gpu), n)
+    values = om.values(k, "mxfp8").to(torch.bfloat16)
+    for t, sign in zip(got, (1, -1)):
+        for at, page in pages.items():
+            some = t[16 * at: 16 * at + 16].cpu()
+            assert torch.equal(some, sign * values[16 * page: 16 * page + len(some)])
+            for empty in (16 * at - 1, 16 * at + 16):
+                if 0 <= empty < n and empty // 16 not in pages:
+                    assert not bool(t[empty].any())
+    del got, t
+    torch.cuda.empty_cache()
