@@ -729,12 +729,12 @@ int mpq_mx_linear(const void* x, int dtype, int64_t ldx, const uint8_t* x_codes,
  *   v_codes  (pages, heads, page / 4, dim / 8, 4, bytes of 8 codes)
  *   v_scales (pages, heads, page / 4, dim / 32, 4)
  * The fourth index of the values is the token within its group of four.  NaN is scale byte 255: the E4M3 codes 0x7f
- * and 0xff under another scale byte, which mpq_kv_write never stores, are not supported (mpq_kv_attend may let such a
- * value reach rows that do not see it).
+ * and 0xff under another scale byte, which mpq_kv_write never stores in a slot of its own, are not supported
+ * (mpq_kv_attend may let such a value reach rows that do not see it).
  *
  * mpq_kv_write: tokens x heads x dim keys and values (MPQ_BF16 or MPQ_F16, strides in elements, dim contiguous)
- * into their slots (page * page size + place in the page); a slot outside the pool is skipped, and of two tokens
- * with one slot either may stay.
+ * into their slots (page * page size + place in the page); a slot outside the pool is skipped.  The other slots of a
+ * call must be distinct: two tokens written to one at once leave a mixture of both (codes of one, scales of the other).
  * mpq_kv_read: sequences' tokens one after the other, `total` of them, sequence i the tokens starts[i] to
  * starts[i + 1] at positions 0, 1, ... of its row of block_table (batch x table_width); zeros where the table
  * names no page of the pool.

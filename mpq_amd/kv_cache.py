@@ -127,7 +127,8 @@ class QuantizedKVCache:
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantise keys and values (tokens, heads, dim; any token and head strides) into ``slots`` (tokens, int64).
-        A slot outside the pool (-1 for padding) is skipped; of two tokens with one slot either may stay."""
+        A slot outside the pool (-1 for padding) is skipped.  The others must be distinct: two tokens written to one slot
+        at once leave a mixture of both there (codes of one under scales of the other)."""
         k, v = self._tokens(k, "k", self.heads), self._tokens(v, "v", self.heads)
         if k.shape != v.shape:
             raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
