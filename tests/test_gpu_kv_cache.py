@@ -518,3 +518,68 @@ def test_read_more_tokens_than_a_launch_has_threads(gpu):
                     assert not bool(t[empty].any())
     del got, t
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("fmt,dtype", [("mxfp8", torch.bfloat16), ("mxfp4", torch.float16)])
+@pytest.mark.parametrize("lens,new,heads,group,page", [
+    ([200, 90], [1, 5], 2, 4, 16),       # 16 rows, one run of keys
+    ([3000, 170], [2, 1], 2, 4, 64),     # 16 rows, runs joined
+    ([300, 130], [100, 70], 2, 2, 16),   # 128 rows
+    ([5000, 300], [60, 3], 1, 4, 32),    # 128 rows, runs joined
+    ([300] * 16, [70] * 16, 8, 4, 32),   # 256 rows
+])
+def test_attend_missing_pages_inside_the_context(gpu, fmt, dtype, lens, new, heads, group, page):
+    """The first page, one in the middle and the last one of a sequence are named wrongly: their positions are seen by no
+    row, against 64 bits."""
+    dim = 128 if heads != 2 else 64
+    b = _Batch(gpu, lens, heads, dim, page, fmt, dtype, seed=3).fill()
+    held, whole = (lens, b.table.clone()), -(-lens[0] // page)
+    for bad, at in ((-1, [whole // 2]), (b.cache.num_pages, [0, whole // 2]), (2 ** 31 - 1, [whole - 1]),
+                    (-(2 ** 31), [0, 1, whole - 1])):
+        b.table = held[1].clone()
+        b.table[0, at] = bad
+        q, starts, (o, lse) = b.attend(new, group, return_lse=True)
+        for i, n in enumerate(lens):
+            hidden = torch.zeros(n, dtype=torch.bool)
+            if i == 0:
+                hidden = torch.isin(torch.arange(n) // page, torch.tensor(at))
+            _compare(b, i, q[starts[i]: starts[i + 1]], o[starts[i]: starts[i + 1]], lse[starts[i]: starts[i + 1]], new[i],
+                     hidden)
+
+
+def _compare(b, i, q, o, lse, new, hidden):
+    """Sequence i against 64 bits, within the bounds of _Batch.check."""
+    dim, u = b.cache.head_dim, UNIT[b.dtype]
+    o, lse = o.cpu().double(), lse.cpu().double()
+    k, v = (om.values(t[b.starts[i]: b.starts[i + 1]], b.fmt) for t in (b.k, b.v))
+    want, wl, pv, mass, big = om.attend(q, k, v, new, dim ** -0.5, True, hidden)
+    delta = (2.0 ** -24 * (dim + 8) * big).unsqueeze(-1)
+    tol = u * want.abs() * 1.01 + (1.01 * u + 2 * delta + 2.0 ** -20) * pv + 1e-30
+    if b.dtype == torch.float16:
+        tol = tol + 2.0 ** -25 * (1 + mass)
+    assert bool(((o - want).abs() <= tol).all()), (i, float(((o - want).abs() / tol).max()))
+    seen = torch.isfinite(wl)
+    assert torch.equal(seen, torch.isfinite(lse)) and bool((lse[~seen] == -math.inf).all())
+    assert bool(((lse - wl)[seen].abs() <= (2.0 ** -20 * (1 + wl.abs()) + 2 * delta.squeeze(-1))[seen]).all())
+
+
+@pytest.mark.parametrize("fmt,dtype,dim", [("mxfp8", torch.bfloat16, 128), ("mxfp4", torch.float16, 64)])
+def test_attend_chunk_beside_single_tokens(gpu, fmt, dtype, dim):
+    """One batch of a chunk, single tokens over long and short contexts and an idle sequence: tiles of 128 rows of which the
+    single tokens fill few, runs that some rows do not reach."""
+    _Batch(gpu, [2100, 700, 1, 1500, 33, 900], 2, dim, 16, fmt, dtype).fill().check([300, 1, 1, 1, 0, 2], 4)
+    _Batch(gpu, [5000, 700, 4000], 1, dim, 16, fmt, dtype).fill().check([40, 1, 1], 4)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+@pytest.mark.parametrize("size", [2.0 ** -24, 2.0 ** -20, 2.0 ** -15])
+@pytest.mark.parametrize("new", [1, 90])
+def test_small_float16_values_are_kept(gpu, fmt, size, new):
+    """A float16 input is a multiple of 2^-24 and so is its quantised value, in at most four significant bits: float16
+    operands hold what a float16 cache was given."""
+    b = _Batch(gpu, [150], 1, 64, 16, fmt, torch.float16)
+    b.k, b.v = (b.k.float() * size).half(), (b.v.float() * size).half()
+    b.fill()
+    for got, x in zip(b.read(), (b.k, b.v)):
+        assert torch.equal(got.cpu(), om.values(x, fmt).half())
+    b.check([new], 2, scale=1.0 / size / 8)
