@@ -583,3 +583,17 @@ def test_small_float16_values_are_kept(gpu, fmt, size, new):
     for got, x in zip(b.read(), (b.k, b.v)):
         assert torch.equal(got.cpu(), om.values(x, fmt).half())
     b.check([new], 2, scale=1.0 / size / 8)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+@pytest.mark.parametrize("lens,new", [([260], [20]), ([3000], [3]), ([260], [150]), ([6000], [60])])
+def test_attend_nan_queries_stay_in_their_rows(gpu, fmt, lens, new):
+    """A NaN or infinite query makes its own row NaN; its neighbours in the tile keep their bits."""
+    b = _Batch(gpu, lens, 2, 64, 16, fmt, torch.bfloat16).fill()
+    q, _, want = b.attend(new, 2)
+    q[1, 3, 5], q[-1, 0, 0] = math.nan, math.inf
+    _, _, got = b.attend(new, 2, q=q)
+    bad = torch.zeros(sum(new), 4, dtype=torch.bool)
+    bad[1, 3], bad[-1, 0] = True, True
+    got, want = got.cpu(), want.cpu()
+    assert bool(got[bad].isnan().all()) and torch.equal(got[~bad], want[~bad])
