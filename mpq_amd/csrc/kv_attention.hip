@@ -7,9 +7,10 @@
 // softmax, in fp32 and base 2.  Scores are formed transposed, S^T = K Q^T: a lane then holds several
 // keys of one row, the row's statistics are per lane, and after exp2 the lane's values are, as they stand, its
 // operand of O^T = V^T P^T: the order of the keys in that product is free, and V^T is loaded in the order in which
-// S^T leaves them.  K and V become 16-bit operands (exact in bf16), P is rounded to 16 bits for the product while
-// its sum is kept in fp32.  The maximum that p is taken against is moved only when a tile exceeds it by more than
-// 2^8: the result does not depend on it, sums and products stay within range, and sums are rarely rescaled.
+// S^T leaves them.  K and V become 16-bit operands (exact for what was written from that type), P is rounded to 16
+// bits for the product while its sum is kept in fp32.  The maximum that p is taken against is moved only when a tile
+// exceeds it by more than 2^8: the result does not depend on it, sums and products stay within range, and sums are
+// rarely rescaled.
 //
 // Positions that a row does not see get -inf; a row that sees nothing is 0 (lse -inf).  Memory behind a sequence's
 // end may hold anything: its scores are replaced and its values read as zeros.  A value block that stands for NaN

@@ -189,10 +189,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const char* __restr
 // read while the ones after it fill.  A row's 16-byte pieces are permuted by bits of its row number, so that the reads
 // of a fragment (one piece of 16 neighbouring rows at a time) fall into all 64 banks.  The scales of 512 values come
 // at once, 16 bytes a row: a die's L2 serves 16 requests of up to 64 bytes a clock, and 4 bytes of each row with
-// every stage took as many requests as the codes (tiles of 256 x 128 ran at 13 requests a clock, 2.7 PFLOP/s).
+// every stage took as many requests as the codes (tiles of 256 x 128 ran at 13 requests a clock, 2.7 PFLOP/s).  In LDS
+// the scale words of a fragment lie 16 bytes apart and do meet in their banks: 36 k of a CU's 97 k LDS cycles.
 //
 // 4096 tokens of mxfp4, 4096 -> 14336: 142 to 163 us on four cards, 2.9 to 3.4 PFLOP/s; 14336 -> 4096, one round of 256
-// tiles: 3.7 to 3.9.  The clock follows the power: on zeros the latter runs at 4.9 PFLOP/s, about what the
+// tiles: 3.5 to 3.9.  The clock follows the power: on zeros the latter runs at 4.9 PFLOP/s, about what the
 // instruction reaches with its operands from LDS and a barrier for every 128 values; with operands in
 // registers it reaches 6.2 to 7.1 PFLOP/s on random data and 8.4 on zeros.  mxfp8, whose instruction reaches 3.7 PFLOP/s:
 // 222 and 185 us, 2.2 and 2.6 PFLOP/s.
